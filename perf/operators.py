@@ -18,17 +18,12 @@ DEV = "cuda"
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
-_loaded = None
-
-
 def _lib():
-    """The package, imported by the first call."""
-    global _loaded
-    if _loaded is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "idol.cpp_amd"))
-        import idolq_lib
-        _loaded = idolq_lib
-    return _loaded
+    path = str(Path(__file__).resolve().parents[1] / "idol.cpp_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import idolq_lib
+    return idolq_lib
 
 
 def listed():
@@ -195,7 +190,7 @@ def prepare(case, seed):
     if case["op"] == "attention":
         for side in ("q", "k"):
             s["cu_" + side] = torch.tensor(_offsets(s["l" + side]), device=DEV, dtype=torch.int32)
-        s["max_q"], s["max_k"] = max(s["lq"]), max(s["lk"])
+        s["max_k"] = max(s["lk"])
     elif case["op"] == "q4":
         s["w"] = s["w"].reshape(-1)
     return s
@@ -275,7 +270,7 @@ def run(s):
         if not own:
             return _attention_plain(s)
         return _lib().attention_packed(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"], c["heads"], c["kv"], c["hd"],
-                                       causal=c["causal"], max_q=s["max_q"], max_k=s["max_k"])
+                                       causal=c["causal"], max_k=s["max_k"])
     if c["op"] == "rotary":
         if not own:
             q = _rotary_plain(s["q"], s, c["heads"])
