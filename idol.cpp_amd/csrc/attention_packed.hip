@@ -265,7 +265,12 @@ struct WaveRows {
             for (int st = 0; st < NS; ++st)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[st][r]);
-            return fmaxf(mx, __shfl_xor(mx, 32)) + Prob<T>::kBias;
+            return fmaxf(mx, __shfl_xor(mx, 32));
+        };
+        // Where a row's reference point goes from m: kBias above its largest score, which lies mx above m. Scores of 2^20 and
+        // more are their own reference point: in fp32 it would not move by kBias, and o and l would lose 2^-24 every tile.
+        auto raise_to = [&](float mx) __attribute__((always_inline)) {
+            return mx + (fabsf(m + mx) < 0x1p20f ? Prob<T>::kBias : 0.0f);
         };
         auto lower = [&](float by) __attribute__((always_inline)) {
             m += by;
@@ -276,7 +281,7 @@ struct WaveRows {
         };
         if (first) {
             const float mx = maximum();
-            lower(mx == -INFINITY ? 0.0f : mx);  // a row without keys keeps weights of 0
+            lower(mx == -INFINITY ? 0.0f : raise_to(mx));  // a row without keys keeps weights of 0
         }
         // the probabilities as MFMA operands (chunk kc: 16 keys) and this lane's sum of them as rounded
         Vec pf[2 * NS];
@@ -301,7 +306,7 @@ struct WaveRows {
         // path: rows with a score more than 2^8 above the reference raise m to their maximum, scale o and l, and the tile's
         // probabilities are taken again. Below that a tile's sum stays under 32 NS 2^8 <= 2^14.
         if (__builtin_amdgcn_ballot_w64(!(lt < (Prob<T>::kBias != 0.0f ? 0x1p-9f : 0x1p15f))) != 0) {
-            const float mx = maximum(), delta = mx > 8.0f ? mx : 0.0f, alpha = __builtin_amdgcn_exp2f(-delta);
+            const float to = raise_to(maximum()), delta = to > 8.0f ? to : 0.0f, alpha = __builtin_amdgcn_exp2f(-delta);
             l *= alpha;
 #pragma unroll
             for (int t = 0; t < kD; ++t)

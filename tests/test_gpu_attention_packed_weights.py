@@ -1,0 +1,36 @@
+"""Packed attention where softmax weights are far apart, through every way that a call can take: row tiles, row tiles cut
+along the keys, key chunks of one launch and divided ones."""
+import pytest
+import torch
+
+import idolq_lib as L
+from test_gpu_attention_packed import BF16, DEV, FP16, check, offsets, oracle
+
+pytestmark = pytest.mark.gpu
+
+WAYS = {  # lq, lk, max_q, max_k: one sequence each
+    "tile": (260, 260, 0, 0), "cut tiles": (150, 2600, 0, 2600), "short": (2, 900, 2, 900),
+    "divided": (1, 9000, 1, 9000), "long": (3, 40000, 3, 40000)}
+
+
+def call(q, k, v, way, **kw):
+    lq, lk, mq, mk = WAYS[way]
+    return L.attention_packed(q, k, v, offsets([lq]).to(DEV), offsets([lk]).to(DEV), 1, 1, q.shape[1], max_q=mq, max_k=mk,
+                              **kw)
+
+
+def rows(n, hd, seed, std=0.0):
+    return torch.randn((n, hd), generator=torch.Generator().manual_seed(seed)) * std
+
+
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("power", [10, 20, 24, 27, 28, 29, 30, 33])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_large_scores_that_tie(way, power, dtype):
+    # every key's score is 2^power exactly (and rounds alike for all keys in base 2): all weights are the same
+    lq, lk = WAYS[way][:2]
+    q, k, v = torch.zeros((lq, 64)), torch.zeros((lk, 64)), rows(lk, 64, 4, 1.0)
+    q[:, 3], k[:, 3] = 2.0 ** 10, 2.0 ** 10
+    q, k, v = (t.to(dtype).to(DEV) for t in (q, k, v))
+    want = v.double().cpu().mean(0).expand(lq, 64)
+    check(call(q, k, v, way, scale=2.0 ** (power - 20)), want, v.double().cpu().abs().mean(0).expand(lq, 64), dtype)
