@@ -15,8 +15,8 @@
 // into LDS (two buffers, 16-byte chunks permuted by row against bank conflicts), one barrier a tile. Scores are taken
 // transposed, S^T = K Q^T on the 32x32x16 matrix instructions, so a lane holds 32 scores of one row; the probabilities
 // become the B operand of O^T = V^T P^T from the registers they are in, and V^T is read out of the row-major V tile by
-// the transposing LDS reads in the key order that the scores have. m is the first tile's maximum and raised only for a
-// tile whose probabilities sum to 2^15 or more. Tiles past a wave's last visible key are skipped, only tiles that some row
+// the transposing LDS reads in the key order that the scores have. m goes by the first tile's maximum and is raised only for
+// a tile with far larger scores. Tiles past a wave's last visible key are skipped, only tiles that some row
 // sees in part are masked. Bound by MFMAs and the softmax's vector work, of which little overlaps: one bf16 prompt of 16384,
 // 32 heads on 8 of 128, 1.9 ms (1.1 PFLOP/s, matrix units busy 60% of the cycles), 8 fp16 prompts of up to 4096, 24 heads of
 // 64, 193 us (0.7; half the products for each exponential). Waves that take the next tile's scores among this tile's
@@ -31,8 +31,11 @@
 // attn_packed_combine merges them in order.
 //
 // Probabilities are rounded to the inputs' type for the matrix product, and the sum l adds the rounded values, so the
-// weights still sum to 1: 2^-9 (bf16) of a weight at most, which averages out below the output's own rounding. With bf16
-// the reference point m lies 2^24 above the row's maximum, so that sums of values near the type's largest stay finite.
+// weights still sum to 1. Each is off by up to 2^-9 (bf16) or 2^-12 (fp16) of itself, so an output by as much of
+// sum p_j |v_j| at most; over values of mean zero that is about what the output's own rounding is (48 sequences in bf16: 2.3e-3
+// of the result in all, 1.7e-3 with fp32 weights). Two bf16 parts a weight would take half as many matrix products again.
+// bf16: m lies 2^24 above the row's maximum, so that sums of values near the type's largest stay finite. fp16: 2^8 below it,
+// as small weights would vanish otherwise (a key 17.5 above 4096 others: a third of their weight).
 #include "q8_dma.h"
 
 #include <algorithm>
@@ -131,14 +134,20 @@ template <typename T>
 struct Prob;
 template <>
 struct Prob<__bf16> {
-    static constexpr float kBias = 24.0f;  // m lies this far above the maximum (fp32 sums of large values stay finite)
+    static constexpr float kBias = 24.0f;   // m lies this far above the maximum (fp32 sums of large values stay finite)
+    static constexpr float kRise = 8.0f;    // a row whose largest score would move m further up than this does so
+    static constexpr float kMost = 0x1p-9f;  // for a lane's sum of a tile that reaches this
     static __device__ __forceinline__ float sum(bf16x2 a, float c) {
         return __builtin_amdgcn_fdot2_f32_bf16(a, bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
     }
 };
 template <>
 struct Prob<_Float16> {
-    static constexpr float kBias = 0.0f;  // fp16 has no exponents to spare
+    // The largest weight is 2^8 or more, so that those down to 2^-22 of it are normal numbers; smaller ones are multiples of
+    // 2^-24, off by at most 2^-25: 2^-33 of the row's sum each.
+    static constexpr float kBias = -8.0f;
+    static constexpr float kRise = 0.0f;
+    static constexpr float kMost = 0x1p15f;
     static __device__ __forceinline__ float sum(f16x2 a, float c) {
         return __builtin_amdgcn_fdot2(a, f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
     }
@@ -302,11 +311,11 @@ struct WaveRows {
             if (NS > 1) lt += ls[NS - 1];
         };
         probabilities();
-        // A lane whose probabilities sum to 2^15 (in m's units) or more, or to inf or NaN, sends the wave through the rare
-        // path: rows with a score more than 2^8 above the reference raise m to their maximum, scale o and l, and the tile's
-        // probabilities are taken again. Below that a tile's sum stays under 32 NS 2^8 <= 2^14.
-        if (__builtin_amdgcn_ballot_w64(!(lt < (Prob<T>::kBias != 0.0f ? 0x1p-9f : 0x1p15f))) != 0) {
-            const float to = raise_to(maximum()), delta = to > 8.0f ? to : 0.0f, alpha = __builtin_amdgcn_exp2f(-delta);
+        // A lane whose probabilities sum to kMost or more (2^7 to 2^15 times the largest that there was), or to inf or NaN,
+        // sends the wave through the rare path: rows whose largest score lies kRise beyond its place below m raise m, scale o
+        // and l, and the tile's probabilities are taken again. Rows that stay have weights of up to 2^8 (bf16: 2^-16).
+        if (__builtin_amdgcn_ballot_w64(!(lt < Prob<T>::kMost)) != 0) {
+            const float to = raise_to(maximum()), delta = to > Prob<T>::kRise ? to : 0.0f, alpha = __builtin_amdgcn_exp2f(-delta);
             l *= alpha;
 #pragma unroll
             for (int t = 0; t < kD; ++t)

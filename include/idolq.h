@@ -204,8 +204,9 @@ size_t idolq_attention_f32_workspace(int64_t batch, int64_t lq, int64_t lk, int6
  * j < lk and, causal, only j <= i + lk - lq (the last query sees every key); the softmax is over scale * (q . k). A query
  * that sees no key gets zeros; what a masked key or value row holds (infinities and NaN too) does not reach the output;
  * output rows outside every sequence are left as they were.
- *   dtype    IDOLQ_BF16 or IDOLQ_F16, of q, k, v and out; probabilities are rounded to it for their product with V, sums
- *            are fp32. head_dim 64 or 128; kv_heads divides heads.
+ *   dtype    IDOLQ_BF16 or IDOLQ_F16, of q, k, v and out; probabilities are rounded to it for their product with V (each off
+ *            by up to 2^-9, fp16 2^-12, of itself; fp16 also by up to 2^-33 of the row's sum, which is more below 2^-22 of
+ *            the largest), sums are fp32. head_dim 64 or 128; kv_heads divides heads.
  *   q, out   [total_q x heads * head_dim], row strides ldq, ldo; k, v [total_k x kv_heads * head_dim], row strides ldk,
  *            ldv; all 16-byte aligned in address and row stride. out must not overlap the inputs.
  *   cu_q, cu_k  seqs + 1 device int32 each, not decreasing. They are read by the kernels only, so a captured call may be

@@ -1,5 +1,7 @@
 """Packed attention where softmax weights are far apart, through every way that a call can take: row tiles, row tiles cut
 along the keys, key chunks of one launch and divided ones."""
+import math
+
 import pytest
 import torch
 
@@ -34,3 +36,22 @@ def test_large_scores_that_tie(way, power, dtype):
     q, k, v = (t.to(dtype).to(DEV) for t in (q, k, v))
     want = v.double().cpu().mean(0).expand(lq, 64)
     check(call(q, k, v, way, scale=2.0 ** (power - 20)), want, v.double().cpu().abs().mean(0).expand(lq, 64), dtype)
+
+
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("gap", [12.0, 15.0, 17.5, 19.0])
+@pytest.mark.parametrize("dtype,hd", [(FP16, 64), (FP16, 128), (BF16, 64)])
+def test_small_weights_next_to_a_dominant_key(way, gap, dtype, hd):
+    # The first key stands `gap` above the others, its values are 0: the output is the small weights' alone. fp16 weights are
+    # multiples of 2^-24 where the largest is 2^8 or more, so each is off by at most 2^-25 / 2^8 = 2^-33 of the row's sum,
+    # beside the relative roundings that check() counts.
+    lq, lk = WAYS[way][:2]
+    q, k, v = rows(lq, hd, 1, 0.3), rows(lk, hd, 2, 0.3), 1 + rows(lk, hd, 3, 0.25)
+    q[:, 0], k[:, 0], k[0, 0] = 4.0, 0.0, gap * math.sqrt(hd) / 4
+    v[0] = 0
+    q, k, v = (t.to(dtype).to(DEV) for t in (q, k, v))
+    o, big = oracle(q, k, v, [lq], [lk], 1, 1, hd, False)
+    if dtype == FP16:
+        # check() allows 2^-13 of `big` among others: what the multiples add is counted as that much more of it
+        big = big + 2.0 ** 13 * 2.0 ** -33 * v.double().cpu().abs().sum(0)
+    check(call(q, k, v, way), o, big, dtype)
