@@ -290,7 +290,9 @@ struct WaveRows {
         };
         if (first) {
             const float mx = maximum();
-            lower(mx == -INFINITY ? 0.0f : raise_to(mx));  // a row without keys keeps weights of 0
+            // A row without keys keeps weights of 0. One whose scores here are all -inf starts far below the scores to come,
+            // so that the first finite ones raise m (as rounded there: 2^-13 in the exponent, as much as an fp16 weight).
+            lower(mx == -INFINITY ? -0x1p12f : raise_to(mx));
         }
         // the probabilities as MFMA operands (chunk kc: 16 keys) and this lane's sum of them as rounded
         Vec pf[2 * NS];

@@ -55,3 +55,24 @@ def test_small_weights_next_to_a_dominant_key(way, gap, dtype, hd):
         # check() allows 2^-13 of `big` among others: what the multiples add is counted as that much more of it
         big = big + 2.0 ** 13 * 2.0 ** -33 * v.double().cpu().abs().sum(0)
     check(call(q, k, v, way), o, big, dtype)
+
+
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("level", [-100.0, -12.0, 0.0, 100.0])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_first_keys_with_scores_of_minus_infinity(way, level, dtype):
+    # keys whose score is -inf have no weight, wherever they are: the first keys of every tile, wave or chunk walk, and
+    # more; the others' scores are near `level`
+    lq, lk = WAYS[way][:2]
+    q, k, v = rows(lq, 64, 5, 0.3), rows(lk, 64, 6, 0.3), rows(lk, 64, 7, 1.0)
+    q[:, 0], k[:, 0], q[:, 1], k[:, 1] = 1.0, 0.0, 32.0, level / 4
+    k[:min(lk - 60, 700), 0] = -math.inf
+    q, k, v = (t.to(dtype).to(DEV) for t in (q, k, v))
+    got = call(q, k, v, way, causal=False)
+    o, big = oracle(q, k, v, [lq], [lk], 1, 1, 64, False)
+    # scores up to 2^8: their fp32 sums are off by up to 2^-15 of them, 2^-7 in the exponent (12: 2^-11; and 2^-13 for the
+    # first finite ones, which are taken 2^12 above the row's reference point)
+    err, u = (got.double().cpu() - o).abs(), torch.finfo(dtype).eps / 2
+    assert (err <= u * o.abs() + (u + (2.0 ** -7 if abs(level) > 12 else 2.0 ** -10)) * (big + o.abs())).all()
+    k[:, 0] = -math.inf
+    assert (call(q, k, v, way) == 0).all()     # nothing has weight
