@@ -363,7 +363,8 @@ struct RowLoader {
 };
 
 // The parts first, first + step, .. of a row merged by 16 lanes (sub: which), HD / 16 columns each: entry(i) is part i's
-// unnormalized columns and its (m, l). Bound by the latency of its loads, so those of eight parts go together and the
+// unnormalized columns and its (m, l); parts without a sum (m = -inf) are left out, others keep what is no number in them
+// whatever their weight. Bound by the latency of its loads, so those of eight parts go together and the
 // maximum is a running one (48 sequences as below, the whole call: 128 us, with a pass for the maximum first 132).
 template <int HD, typename F>
 __device__ __forceinline__ void merge_parts(const PackedParams& p, int first, int step, int parts, int sub, F&& entry,
@@ -392,15 +393,15 @@ __device__ __forceinline__ void merge_parts(const PackedParams& p, int first, in
         const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
         m = to, l *= keep;
 #pragma unroll
-        for (int c = 0; c < N; ++c) o[c] = keep == 0.0f ? 0.0f : o[c] * keep;
+        for (int c = 0; c < N; ++c) o[c] *= keep;
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-            if (e[u].x == -INFINITY) continue;
-            const float wgt = __builtin_amdgcn_exp2f(e[u].x - m);
-            l = fmaf(wgt, e[u].y, l);
+            const bool none = e[u].x == -INFINITY;  // (selects, no branch: the loads of all eight stay in front of it)
+            const float wgt = none ? 0.0f : __builtin_amdgcn_exp2f(e[u].x - m);
+            l = fmaf(wgt, none ? 0.0f : e[u].y, l);
             const float* const f = reinterpret_cast<const float*>(v[u]);
 #pragma unroll
-            for (int c = 0; c < N; ++c) o[c] = wgt == 0.0f ? o[c] : fmaf(wgt, f[c], o[c]);
+            for (int c = 0; c < N; ++c) o[c] = fmaf(wgt, none ? 0.0f : f[c], o[c]);
         }
     }
 }
@@ -728,11 +729,11 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : HD == 64 ? 3 : 2) void a
             for (int i = 0; i < NW; ++i) mx = fmaxf(mx, red_m[i][r]);
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-                const float wgt = red_m[i][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(red_m[i][r] - mx);
+                if (red_m[i][r] == -INFINITY) continue;
+                const float wgt = __builtin_amdgcn_exp2f(red_m[i][r] - mx);
                 sum = fmaf(wgt, red_l[i][r], sum);
 #pragma unroll
-                for (int d = 0; d < N; ++d)
-                    f[d] = wgt == 0.0f ? f[d] : fmaf(wgt, red[(i * 32 + r) * kPitch + piece * N + d], f[d]);
+                for (int d = 0; d < N; ++d) f[d] = fmaf(wgt, red[(i * 32 + r) * kPitch + piece * N + d], f[d]);
             }
             if (parts == 1) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -788,10 +789,11 @@ __global__ __launch_bounds__(256) void attn_packed_combine(PackedParams p) {
 #pragma unroll
         for (int c = 0; c < N; ++c) o[c] = 0.0f;
         for (int g = 0; g < G; ++g) {
-            const float wgt = red_m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(red_m[g] - m);
+            if (red_m[g] == -INFINITY) continue;
+            const float wgt = __builtin_amdgcn_exp2f(red_m[g] - m);
             l = fmaf(wgt, red_l[g], l);
 #pragma unroll
-            for (int c = 0; c < N; ++c) o[c] = wgt == 0.0f ? o[c] : fmaf(wgt, red_o[g][sub * N + c], o[c]);
+            for (int c = 0; c < N; ++c) o[c] = fmaf(wgt, red_o[g][sub * N + c], o[c]);
         }
     }
     const int tk = r / p.group;

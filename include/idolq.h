@@ -202,7 +202,8 @@ size_t idolq_attention_f32_workspace(int64_t batch, int64_t lq, int64_t lk, int6
  * k_lens[s] of these: a cache gives each sequence rows to grow into); query head h (columns
  * [h * head_dim, (h + 1) * head_dim) of q and out) reads key head h / (heads / kv_heads). Query i of lq sees the keys
  * j < lk and, causal, only j <= i + lk - lq (the last query sees every key); the softmax is over scale * (q . k). A query
- * that sees no key, or only keys with scores of -inf, gets zeros; what a masked key or value row holds (infinities and NaN too) does not reach the output;
+ * that sees no key, or only keys with scores of -inf, gets zeros; what a masked key or value row holds (infinities and NaN too) does not reach the output; one
+ * in a value row that a query sees with any score but -inf makes that column of the query no number (an infinity or NaN);
  * output rows outside every sequence are left as they were.
  *   dtype    IDOLQ_BF16 or IDOLQ_F16, of q, k, v and out; probabilities are rounded to it for their product with V (each off
  *            by up to 2^-9, fp16 2^-12, of itself; fp16 also by up to 2^-33 of the row's sum, which is more below 2^-22 of

@@ -76,3 +76,21 @@ def test_first_keys_with_scores_of_minus_infinity(way, level, dtype):
     assert (err <= u * o.abs() + (u + (2.0 ** -7 if abs(level) > 12 else 2.0 ** -10)) * (big + o.abs())).all()
     k[:, 0] = -math.inf
     assert (call(q, k, v, way) == 0).all()     # nothing has weight
+
+
+@pytest.mark.parametrize("way", ["cut tiles", "short", "divided", "long"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_value_that_is_no_number_is_seen_behind_any_weight(way, bad, dtype):
+    # the keys from 384 on have scores 200 below the others, so whole waves and parts have no weight in the sum
+    lq, lk = WAYS[way][:2]
+    q, k, v = rows(lq, 64, 8, 0.3), rows(lk, 64, 9, 0.3), rows(lk, 64, 10, 1.0)
+    q[:, 0], k[:, 0] = 16.0, 0.0
+    k[384:, 0] = -100.0
+    q, k, v = (t.to(dtype).to(DEV) for t in (q, k, v))
+    clean = call(q, k, v, way)
+    v[lk * 2 // 3 if lk > 1000 else 390, 5] = bad
+    got = call(q, k, v, way)
+    assert not torch.isfinite(got[:, 5]).any()
+    others = [c for c in range(64) if c != 5]
+    assert torch.equal(got[:, others], clean[:, others]) and torch.isfinite(clean).all()
