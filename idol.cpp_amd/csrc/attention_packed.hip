@@ -51,6 +51,7 @@ constexpr int kTilePart = 256;  // least keys of a part
 constexpr int kFewRows = 64;    // sequences of up to so many rows go to attn_packed_few where both kernels run
 constexpr int kFewKeys = 32;    // keys of a wave's tile there
 constexpr int kFewWaves = 4;
+constexpr int64_t kListBytes = (int64_t)64 << 20;
 
 struct PackedParams {
     const void* q;
@@ -70,6 +71,7 @@ struct PackedParams {
     int chunk;         // attn_packed_few: keys of a chunk
     int per;           // and entries of a sequence (its last chunk takes the rest); 0: as many as its rows' chunks
     int part_rows;     // rows a sequence may have to be cut into parts
+    int sparse;        // the parts' entries go by their keys, not by the list (see first_part)
     float* parts;      // O [entry][HD] of the parts' rows, then (m, l) [entry]
     int64_t part_count;
     int tile_chunk, tile_parts;  // attn_packed_tile: keys of a part, at most so many parts (1: none is cut)
@@ -631,6 +633,12 @@ __device__ __forceinline__ int parts_of(const PackedParams& p, int64_t rows, int
 __device__ __forceinline__ int64_t first_chunk(const PackedParams& p, int s, int first_key) {
     return p.per ? (int64_t)s * p.per : (int64_t)first_key / p.chunk + s;
 }
+// The first part's entry in the workspace, of a sequence that is cut: its first chunk's, or, where few of many sequences can
+// be cut, the half chunk that its first key is in. (A cut sequence has more than one chunk of keys, x > 1 chunks, and
+// takes ceil(x) <= floor(2 x) entries, so it ends before the next one's first.)
+__device__ __forceinline__ int64_t first_part(const PackedParams& p, int s, int first_key) {
+    return p.sparse ? 2 * (int64_t)first_key / p.chunk : first_chunk(p, s, first_key);
+}
 
 // NW waves: 4 for long key ranges, so that a CU holds two or three workgroups and one's loads, start and merge pass under the
 // others' work (48 sequences of up to 8192 keys, 32 heads on 8 of 128: 117 us in this kernel, 4.8 TB/s; one workgroup a CU
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : HD == 64 ? 3 : 2) void a
                     *reinterpret_cast<uint32_t*>(out + d) = __builtin_bit_cast(uint32_t, __builtin_convertvector(g, typename PipeMfma<T>::pair));
                 }
             } else {
-                const int64_t to = (slot * p.kv_heads + kvh) * p.part_rows + at;
+                const int64_t to = ((first_part(p, s, rk.first) + part) * p.kv_heads + kvh) * p.part_rows + at;
 #pragma unroll
                 for (int d = 0; d < N; d += 2)
                     *reinterpret_cast<float2*>(p.parts + to * HD + piece * N + d) = make_float2(f[d], f[d + 1]);
@@ -759,22 +767,31 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : HD == 64 ? 3 : 2) void a
 }
 
 // Merges the parts of the sequences that attn_packed_few cut. G groups of 16 lanes take every G-th part of a row each (few
-// rows of many parts: G = 16, a workgroup a row), and their sums are added in order through LDS.
-template <typename T, int HD, int G>
+// rows of many parts: G = 16, a workgroup a row), and their sums are added in order through LDS. SPARSE: a workgroup takes 16
+// rows of an entry and works where a sequence's parts begin there.
+template <typename T, int HD, int G, bool SPARSE>
 __global__ __launch_bounds__(256) void attn_packed_combine(PackedParams p) {
+    static_assert(!SPARSE || G == 1);
     constexpr int N = HD / 16;
     __shared__ float red_o[G > 1 ? G : 1][HD], red_m[G], red_l[G];
     const int grp = threadIdx.x >> 4, sub = threadIdx.x & 15;
     const int64_t id = G > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 16 + grp;  // (sequence, key head, row)
-    const int r = (int)(id % p.part_rows), kvh = (int)(id / p.part_rows % p.kv_heads);
-    const int64_t sq = id / p.part_rows / p.kv_heads;
+    int r = (int)(id % p.part_rows), kvh = (int)(id / p.part_rows % p.kv_heads);
+    int64_t sq = id / p.part_rows / p.kv_heads;
+    if constexpr (SPARSE) {  // (entry, key head, rows / 16)
+        const int blocks = pieces(p.part_rows, 16);
+        r = (int)blockIdx.x % blocks * 16 + grp, kvh = (int)blockIdx.x / blocks % p.kv_heads;
+        const int64_t entry = (int)blockIdx.x / blocks / p.kv_heads;
+        sq = find_sequence(p.seqs, entry, [&](int i) { return first_part(p, i, clamped(p.cu_k, i, p.total_k)); });
+        if (first_part(p, (int)sq, clamped(p.cu_k, (int)sq, p.total_k)) != entry) return;
+    }
     if (sq >= p.seqs) return;
     const int s = (int)sq;
     const Rows rq = rows_of(p.cu_q, s, p.total_q), rk = keys_of(p, s);
     const int64_t rows = (int64_t)rq.count * p.group;
     const int parts = parts_of(p, rows, rk.count);
     if (r >= rows || rows > p.few_rows || parts == 1) return;
-    const int64_t first = first_chunk(p, s, rk.first) * p.kv_heads + kvh;  // part i: entry first + i kv_heads
+    const int64_t first = first_part(p, s, rk.first) * p.kv_heads + kvh;  // part i: entry first + i kv_heads
     auto entry = [&](int i) { return (first + (int64_t)i * p.kv_heads) * p.part_rows + r; };
     float o[N], m, l;
     merge_parts<HD>(p, G > 1 ? grp : 0, G, parts, sub, entry, o, m, l);
@@ -828,9 +845,18 @@ struct PackedPlan {
     int64_t part_rows;  // 0: no sequence is cut
     int64_t entries;    // chunks
     int64_t per;        // of a sequence, or 0
+    int64_t part_entries;  // the workspace's entries for parts of chunks
+    bool sparse;        // they go by half chunks of keys
     int64_t tile_chunk, tile_parts;  // attn_packed_tile's keys of a part and parts (1: none is cut)
     int64_t few_entries, tile_entries;  // rows of parts in the workspace
     size_t bytes;       // workspace
+
+    int64_t sparse_grid(int64_t kv_heads) const { return part_entries * kv_heads * ((part_rows + 15) / 16); }
+    // whether every launch stays below 2^31 threads
+    bool fits(int64_t seqs, int64_t kv_heads) const {
+        return std::max({slots * kv_heads, entries * kv_heads, sparse ? sparse_grid(kv_heads) : seqs * kv_heads * part_rows}) <=
+               0x7fffffff / 256;
+    }
 };
 PackedPlan packed_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t max_q, int64_t max_k, int64_t heads,
                        int64_t kv_heads, int64_t head_dim, bool workspace) {
@@ -859,7 +885,7 @@ PackedPlan packed_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t m
             int64_t chunk = std::max<int64_t>((tiles * keys / room + kTileKeys - 1) / kTileKeys * kTileKeys, kTilePart);
             w.tile_parts = std::max<int64_t>((max_k + chunk - 1) / chunk, 1);
             // One long sequence among many short ones needs parts of its own length only: the row tiles together get up to
-            // eight parts for every place on the device (270 MB of workspace), 64 each at most.
+            // eight parts for every place on the device (up to 270 MB of workspace for these), 64 each at most.
             const int64_t most = std::max<int64_t>(std::min<int64_t>(8 * room / (w.slots * kv_heads), 64), 1);
             if (w.tile_parts > most) {
                 w.tile_parts = most;
@@ -884,9 +910,17 @@ PackedPlan packed_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t m
         w.entries = total_k / w.chunk + seqs;
         const int64_t per = std::max<int64_t>((max_k + w.chunk - 1) / w.chunk, 1);
         if (per <= w.entries / seqs) w.per = per, w.entries = seqs * per;
+        // Only sequences of more than one chunk have parts, but the list gives every sequence part_rows rows of the workspace
+        // (20000 sequences, 32 heads on 8 of 128, no bounds: 5.4 GB). Where that passes kListBytes the entries go by half
+        // chunks of keys, 2 total_k / chunk + 1, if they are fewer: 2048 / kv_heads + 1 at most, 70 MB with 64 rows of 128 values.
+        const int64_t halves = 2 * total_k / w.chunk + 1;
+        w.sparse = w.entries * kv_heads * w.part_rows * (head_dim + 2) * 4 > kListBytes && halves < w.entries;
+        w.part_entries = w.sparse ? halves : w.entries;
     }
-    w.few_entries = w.entries * kv_heads * w.part_rows;
+    w.few_entries = w.part_entries * kv_heads * w.part_rows;
     w.bytes = (size_t)(w.few_entries + w.tile_entries) * (size_t)(head_dim + 2) * 4;
+    // (without parts there may be fewer chunks)
+    if (workspace && !w.fits(seqs, kv_heads)) return packed_plan(seqs, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, false);
     return w;
 }
 
@@ -910,10 +944,12 @@ int run(PackedParams p, const PackedPlan& w, hipStream_t s) {
         if (int rc = check_launch("attn_packed_few")) return rc;
         if (w.part_rows) {
             const int64_t rows = (int64_t)p.seqs * p.kv_heads * w.part_rows;
-            if (w.many_parts)
-                hipLaunchKernelGGL((attn_packed_combine<T, HD, 16>), dim3((unsigned)rows), dim3(256), 0, s, p);
+            if (w.sparse)
+                hipLaunchKernelGGL((attn_packed_combine<T, HD, 1, true>), dim3((unsigned)w.sparse_grid(p.kv_heads)), dim3(256), 0, s, p);
+            else if (w.many_parts)
+                hipLaunchKernelGGL((attn_packed_combine<T, HD, 16, false>), dim3((unsigned)rows), dim3(256), 0, s, p);
             else
-                hipLaunchKernelGGL((attn_packed_combine<T, HD, 1>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, p);
+                hipLaunchKernelGGL((attn_packed_combine<T, HD, 1, false>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, p);
             return check_launch("attn_packed_combine");
         }
     }
@@ -958,9 +994,7 @@ extern "C" int idolq_attention_packed(const void* q, const void* k, const void* 
     PackedPlan w = packed_plan(seqs, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, true);
     if (w.bytes && (!workspace || workspace_bytes < w.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
         w = packed_plan(seqs, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, false);
-    if (w.slots * kv_heads > 0x7fffffff / 256 || w.entries * kv_heads > 0x7fffffff / 256 ||
-        seqs * kv_heads * w.part_rows > 0x7fffffff / 256)
-        return fail(IDOLQ_EINVAL, "packed attention: too many sequences, rows or heads");
+    if (!w.fits(seqs, kv_heads)) return fail(IDOLQ_EINVAL, "packed attention: too many sequences, rows or heads");
     if (out == q || out == k || out == v) return fail(IDOLQ_EINVAL, "packed attention: out must not overlap q, k or v");
     PackedParams p{};
     p.q = q, p.k = k, p.v = v, p.out = out, p.cu_q = cu_q, p.cu_k = cu_k, p.k_lens = k_lens;
@@ -971,7 +1005,7 @@ extern "C" int idolq_attention_packed(const void* q, const void* k, const void* 
     p.scale_log2 = scale * 1.4426950408889634f;
     p.ordered = seqs > 1 && seqs <= kOrdered && w.tile_parts == 1;
     p.slots = (int)w.slots, p.few_rows = w.few_rows, p.chunk = (int)std::min<int64_t>(w.chunk, 0x7fffffff);
-    p.part_rows = (int)w.part_rows, p.per = (int)w.per;
+    p.part_rows = (int)w.part_rows, p.per = (int)w.per, p.sparse = w.sparse;
     p.parts = static_cast<float*>(workspace);
     p.part_count = w.few_entries + w.tile_entries;
     p.tile_chunk = (int)w.tile_chunk, p.tile_parts = (int)w.tile_parts, p.tile_entry = w.few_entries;
