@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
 #include <string>
@@ -41,6 +42,30 @@ int fail(int code, const std::string& msg);
 int check_launch(const char* what);
 inline bool dtype_ok(int dt) { return dt == IDOLQ_F32 || dt == IDOLQ_F16 || dt == IDOLQ_BF16; }
 inline size_t dtype_size(int dt) { return dt == IDOLQ_F32 ? 4 : 2; }
+
+// Rows of a strided buffer, all in bytes.
+struct RowBlock {
+    const void* p;
+    int64_t rows, ld, width;  // ld >= width
+};
+// Whether two of them share a byte: columns of one buffer (the same stride) are told apart without a look at the rows, others
+// by the rows of the shorter block where their ranges meet at all.
+inline bool rows_overlap(RowBlock a, RowBlock b) {
+    if (a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+    if (d >= (a.rows - 1) * a.ld + a.width || -d >= (b.rows - 1) * b.ld + b.width) return false;
+    auto below = [](int64_t n, int64_t by) { return n / by - (n % by < 0); };  // floor(n / by)
+    if (a.ld == b.ld) {  // rows i of a and i + k of b: -b.width < d + k ld < a.width
+        const int64_t k = std::max(below(-b.width - d, a.ld) + 1, 1 - a.rows);
+        return k < b.rows && d + k * a.ld < a.width;
+    }
+    if (a.rows > b.rows) return rows_overlap(b, a);
+    for (int64_t i = 0; i < a.rows; ++i) {
+        const int64_t j = std::max<int64_t>(below(i * a.ld - d - b.width, b.ld) + 1, 0);
+        if (j < b.rows && d + j * b.ld < i * a.ld + a.width) return true;
+    }
+    return false;
+}
 
 // ------------------------------------------------------------------------------------------------ device: dtypes
 __device__ __forceinline__ float half_bits_to_float(uint16_t h) {

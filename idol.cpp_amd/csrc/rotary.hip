@@ -228,6 +228,16 @@ extern "C" int idolq_rotary(const void* x, void* y, int dtype, int64_t rows, int
     if (rows == 0) return IDOLQ_OK;
     if (!x || !y || !pos || !freqs || (heads2 && (!x2 || !y2)))
         return fail(IDOLQ_EINVAL, "rotary buffers must be non-null");
+    const int64_t bytes = (int64_t)dtype_size(dtype), second = heads2 ? rows : 0;
+    const RowBlock in[2] = {{x, rows, ldx * bytes, heads * head_dim * bytes}, {x2, second, ldx2 * bytes, heads2 * head_dim * bytes}};
+    const RowBlock to[2] = {{y, rows, ldy * bytes, heads * head_dim * bytes}, {y2, second, ldy2 * bytes, heads2 * head_dim * bytes}};
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2; ++j) {
+            const bool in_place = i == j && to[i].p == in[j].p && (to[i].ld == in[j].ld || rows == 1);
+            if (!in_place && rows_overlap(to[i], in[j]))
+                return fail(IDOLQ_EINVAL, "rotary outputs must not overlap inputs, but for each its own in place");
+        }
+    if (rows_overlap(to[0], to[1])) return fail(IDOLQ_EINVAL, "rotary outputs must not overlap");
     p.x[0] = x, p.x[1] = x2, p.y[0] = y, p.y[1] = y2;
     p.ldx[0] = ldx, p.ldx[1] = ldx2, p.ldy[0] = ldy, p.ldy[1] = ldy2;
     p.heads[0] = (int)heads, p.heads[1] = (int)heads2;
@@ -236,11 +246,10 @@ extern "C" int idolq_rotary(const void* x, void* y, int dtype, int64_t rows, int
     p.inverse = (flags & IDOLQ_ROTARY_INVERSE) != 0;
     const bool inter = (flags & IDOLQ_ROTARY_INTERLEAVED) != 0;
     // the largest power of two of elements (up to 8) that divides every stride, address, the pairs and what is copied
-    const int64_t size = (int64_t)dtype_size(dtype);
     int64_t bits = (inter ? 2 * pairs : pairs) | head_dim | (head_dim - 2 * pairs) | ldx | ldy | 8;
-    bits |= (int64_t)(reinterpret_cast<uintptr_t>(x) / size) | (int64_t)(reinterpret_cast<uintptr_t>(y) / size);
+    bits |= (int64_t)(reinterpret_cast<uintptr_t>(x) / bytes) | (int64_t)(reinterpret_cast<uintptr_t>(y) / bytes);
     if (heads2)
-        bits |= ldx2 | ldy2 | (int64_t)(reinterpret_cast<uintptr_t>(x2) / size) | (int64_t)(reinterpret_cast<uintptr_t>(y2) / size);
+        bits |= ldx2 | ldy2 | (int64_t)(reinterpret_cast<uintptr_t>(x2) / bytes) | (int64_t)(reinterpret_cast<uintptr_t>(y2) / bytes);
     const int64_t step = bits & -bits;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == IDOLQ_F32) return inter ? dispatch<IDOLQ_F32, true>(p, step, s) : dispatch<IDOLQ_F32, false>(p, step, s);

@@ -238,7 +238,8 @@ enum { IDOLQ_ROTARY_INTERLEAVED = 1, IDOLQ_ROTARY_INVERSE = 2 };
  * by axis 1 and so on. A pair is elements (j, j + P) of the head, with IDOLQ_ROTARY_INTERLEAVED (2 j, 2 j + 1); elements
  * from 2 P on are copied. IDOLQ_ROTARY_INVERSE turns by -t: the inverse, and the gradient of the forward call.
  *   x, y     [rows x heads * head_dim], row strides ldx, ldy; y may be x (same stride), else they must not overlap
- *   x2, y2   a second tensor turned by the same positions (the keys) in the same launch; heads2 = 0 for none
+ *   x2, y2   a second tensor turned by the same positions (the keys) in the same launch; heads2 = 0 for none. y2 may be x2;
+ *            other overlaps of an output with an input or the other output are refused
  *   head_dim 2 to 256; any strides and alignment (16-byte accesses where addresses, strides and sections allow them)
  *   pos      [rows x axes] of pos_kind IDOLQ_POS_I32, IDOLQ_POS_I64 or IDOLQ_POS_F32, row stride ldp; freqs [P] fp32
  * The angle is formed and reduced in fp64, so far positions keep fp32's accuracy.

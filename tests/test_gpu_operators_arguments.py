@@ -1,0 +1,35 @@
+"""Views of one buffer that the packed attention, rotary and 4-bit product calls take as inputs and outputs, and those that
+they refuse because an output overlaps an input."""
+import pytest
+import torch
+
+import idolq_lib as L
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+BF16 = torch.bfloat16
+
+
+def rows(n, cols, seed):
+    return torch.randn((n, cols), generator=torch.Generator().manual_seed(seed)).to(BF16).to(DEV)
+
+
+def test_rotary_between_columns_and_rows_of_one_buffer():
+    pos = torch.arange(9, dtype=torch.int32, device=DEV)[:, None] * 7
+    freqs = torch.linspace(1, 0.01, 16, device=DEV)
+    turn = lambda x, k=None, **kw: L.rotary(x, 4, 64, pos, freqs, [16], k=k, kv_heads=0 if k is None else 2, **kw)  # noqa: E731
+    wide = rows(9, 1024, 1)
+    x, k = wide[:, :256], wide[:, 256:384]
+    want_x, want_k = turn(x.contiguous(), k.contiguous())
+    turn(x, k, out=wide[:, 384:640], k_out=wide[:, 640:768])
+    assert torch.equal(wide[:, 384:640], want_x) and torch.equal(wide[:, 640:768], want_k)
+    turn(x, k, out=x, k_out=k)
+    assert torch.equal(x, want_x) and torch.equal(k, want_k)
+    tall = rows(27, 256, 2)
+    want = turn(tall[::3].contiguous())
+    turn(tall[::3], out=tall[1::3])
+    assert torch.equal(tall[1::3], want)
+    with pytest.raises(ValueError, match="overlap"):
+        turn(tall[:9], out=tall[1:10])
+    with pytest.raises(ValueError, match="overlap"):
+        turn(x, k, out=wide[:, 256:512])

@@ -3,7 +3,7 @@ buffers that overlap. Every call below is refused before anything is launched (t
 import pytest
 
 import idolq_lib as L
-from test_operators_host import P, attention
+from test_operators_host import P, attention, rotary
 
 
 def workspace(seqs, total_q, total_k, max_q, max_k, heads, kv_heads, hd):
@@ -26,3 +26,16 @@ def test_packed_attention_takes_as_many_sequences_with_a_workspace_as_without(se
     for ws, size in ((None, 0), (P, 2 ** 40)):
         assert attention(**over, ws=ws, ws_bytes=size) == L.EINVAL
         assert b"overlap" in L.load().idolq_last_error(), L.load().idolq_last_error()
+
+
+A, B, C, D = 0x100000, 0x200000, 0x300000, 0x400000    # far apart
+
+
+@pytest.mark.parametrize("over", [
+    dict(x=A, y=A, ldx=256, ldy=264), dict(x2=C, y2=C, ldx2=128, ldy2=256), dict(x=A, y=A + 16), dict(x=A, y=A - 512 * 3),
+    dict(y=C), dict(y2=A), dict(y2=B), dict(y2=B + 512 * 2 + 510), dict(x=A, y=A + 256, ldx=512, ldy=512),
+    dict(x=A, y=A + 1024 * 3, ldx=512, ldy=256), dict(x=A, y=A, ldx=512, ldy=512, x2=A + 512, y2=A + 510, ldx2=512, ldy2=512)])
+def test_rotary_refuses_overlapping_outputs(over):
+    # four rows of 256 elements in bf16 (x, y) and of 128 (x2, y2)
+    assert rotary(**{**dict(x=A, y=B, x2=C, y2=D), **over}) == L.EINVAL
+    assert b"overlap" in L.load().idolq_last_error(), L.load().idolq_last_error()
