@@ -995,7 +995,10 @@ extern "C" int idolq_attention_packed(const void* q, const void* k, const void* 
     if (w.bytes && (!workspace || workspace_bytes < w.bytes || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
         w = packed_plan(seqs, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, false);
     if (!w.fits(seqs, kv_heads)) return fail(IDOLQ_EINVAL, "packed attention: too many sequences, rows or heads");
-    if (out == q || out == k || out == v) return fail(IDOLQ_EINVAL, "packed attention: out must not overlap q, k or v");
+    const RowBlock to{out, total_q, ldo * 2, heads * head_dim * 2};
+    if (rows_overlap(to, {q, total_q, ldq * 2, heads * head_dim * 2}) || rows_overlap(to, {k, total_k, ldk * 2, kv_heads * head_dim * 2}) ||
+        rows_overlap(to, {v, total_k, ldv * 2, kv_heads * head_dim * 2}))
+        return fail(IDOLQ_EINVAL, "packed attention: out must not overlap q, k or v");
     PackedParams p{};
     p.q = q, p.k = k, p.v = v, p.out = out, p.cu_q = cu_q, p.cu_k = cu_k, p.k_lens = k_lens;
     p.ldq = ldq, p.ldk = ldk, p.ldv = ldv, p.ldo = ldo;

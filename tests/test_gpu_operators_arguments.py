@@ -33,3 +33,15 @@ def test_rotary_between_columns_and_rows_of_one_buffer():
         turn(tall[:9], out=tall[1:10])
     with pytest.raises(ValueError, match="overlap"):
         turn(x, k, out=wide[:, 256:512])
+
+
+def test_packed_attention_into_columns_between_its_inputs():
+    wide = rows(50, 1024, 3)
+    q, k, v, out = wide[:, :256], wide[:, 256:384], wide[:, 640:768], wide[:, 384:640]
+    cu = torch.tensor([0, 30, 50], dtype=torch.int32, device=DEV)
+    want = L.attention_packed(q, k, v, cu, cu, 4, 2, 64, causal=True)
+    L.attention_packed(q, k, v, cu, cu, 4, 2, 64, causal=True, out=out)
+    assert torch.equal(out, want)
+    for bad in (wide[:, 200:456], wide[:, 512:768], wide[:, 8:264]):
+        with pytest.raises(ValueError, match="overlap"):
+            L.attention_packed(q, k, v, cu, cu, 4, 2, 64, causal=True, out=bad)

@@ -39,3 +39,12 @@ def test_rotary_refuses_overlapping_outputs(over):
     # four rows of 256 elements in bf16 (x, y) and of 128 (x2, y2)
     assert rotary(**{**dict(x=A, y=B, x2=C, y2=D), **over}) == L.EINVAL
     assert b"overlap" in L.load().idolq_last_error(), L.load().idolq_last_error()
+
+
+@pytest.mark.parametrize("over", [
+    dict(out=A + 16), dict(out=A - 512 * 7), dict(out=C), dict(out=D), dict(out=C + 256 * 8 + 240), dict(out=C - 512 * 7 - 496),
+    dict(out=A + 512, ldq=1024, ldo=264), dict(out=A + 1024 - 16, ldq=512, ldo=512)])
+def test_packed_attention_refuses_outputs_over_its_inputs(over):
+    # eight rows of 256 elements (q, out), nine of 128 (k, v)
+    assert attention(**{**dict(q=A, k=C, v=D), **over}) == L.EINVAL
+    assert b"overlap" in L.load().idolq_last_error(), L.load().idolq_last_error()
