@@ -465,6 +465,14 @@ extern "C" int idolq_q4_gemv(const void* x, int x_dtype, int64_t m, int64_t k, i
     if (bias) p.bias = static_cast<const char*>(bias) + n_offset * (int64_t)dtype_size(bias_dtype);
     if (reinterpret_cast<uintptr_t>(p.w) % (kind == IDOLQ_KIND_Q4_0 ? 2 : 16) != 0)
         return fail(IDOLQ_EINVAL, "Q4_0 blocks must be 2-byte aligned, Q4_K blocks 16-byte aligned");
+    // y is written while others still read x; a residual's element is read by the thread that writes y's in its place
+    const int64_t xs = (int64_t)dtype_size(x_dtype), ys = (int64_t)dtype_size(y_dtype);
+    const RowBlock to{y, m, ldy * ys, n * ys};
+    if (rows_overlap(to, {x, m, ldx * xs, k * xs})) return fail(IDOLQ_EINVAL, "y must not overlap x");
+    if (residual && !(residual == y && residual_dtype == y_dtype && (ldr == ldy || m == 1))) {
+        const int64_t rs = (int64_t)dtype_size(residual_dtype);
+        if (rows_overlap(to, {residual, m, ldr * rs, n * rs})) return fail(IDOLQ_EINVAL, "y must not overlap the residual, unless it is y");
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
     return kind == IDOLQ_KIND_Q4_0 ? by_type<IDOLQ_KIND_Q4_0>(p, x_dtype, s) : by_type<IDOLQ_KIND_Q4_K>(p, x_dtype, s);
 }

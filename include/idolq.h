@@ -314,7 +314,8 @@ int idolq_q4_k_gemm(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ld
  * 0.5625 a weight. x is bf16, fp16 or fp32 of any stride and alignment, with finite values (an infinite activation makes
  * its row NaN). EXACT arithmetic: the codes enter the products as they are and each group of 32 is scaled in fp32
  * (idolq_q8_0_gemm's and idolq_q4_k_gemm's DEQUANT rounds each weight to x's type first). bias, residual, act, y and the
- * flag IDOLQ_FLAG_ROUND_BEFORE_BIAS as idolq_q8_0_gemm; no workspace.
+ * flag IDOLQ_FLAG_ROUND_BEFORE_BIAS as idolq_q8_0_gemm; no workspace. The residual may be y itself (same stride and type);
+ * y must not overlap it otherwise, nor x.
  * Small-m form of the Q4_0 and Q4_K cases of tools/idol_triton.py:48-82. */
 int idolq_q4_gemv(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const uint8_t* w, int kind,
                   int64_t n_total, int64_t n_offset, int64_t n, const void* bias, int bias_dtype, const void* residual,

@@ -45,3 +45,20 @@ def test_packed_attention_into_columns_between_its_inputs():
     for bad in (wide[:, 200:456], wide[:, 512:768], wide[:, 8:264]):
         with pytest.raises(ValueError, match="overlap"):
             L.attention_packed(q, k, v, cu, cu, 4, 2, 64, causal=True, out=bad)
+
+
+def test_q4_gemv_into_its_residual_and_columns_next_to_its_inputs():
+    w = torch.randint(0, 256, (64 * 8 * 18,), generator=torch.Generator().manual_seed(4), dtype=torch.uint8).reshape(-1, 18)
+    w[:, :2] = torch.tensor([0.03], dtype=torch.float16).view(torch.uint8)
+    w = w.reshape(-1).to(DEV)
+    wide = rows(7, 512, 5)
+    x, res = wide[:, :256], wide[:, 256:320]
+    call = lambda **kw: L.q4_gemv(x, w, L.KIND_Q4_0, 64, residual=res, **kw)  # noqa: E731
+    want = call()
+    call(out=wide[:, 320:384])
+    assert torch.equal(wide[:, 320:384], want)
+    call(out=res)
+    assert torch.equal(res, want)
+    for bad in (wide[:, 200:264], wide[:, 250:314], wide[:, 8:72]):
+        with pytest.raises(ValueError, match="overlap"):
+            call(out=bad)

@@ -3,7 +3,7 @@ buffers that overlap. Every call below is refused before anything is launched (t
 import pytest
 
 import idolq_lib as L
-from test_operators_host import P, attention, rotary
+from test_operators_host import P, attention, gemv, rotary
 
 
 def workspace(seqs, total_q, total_k, max_q, max_k, heads, kv_heads, hd):
@@ -47,4 +47,13 @@ def test_rotary_refuses_overlapping_outputs(over):
 def test_packed_attention_refuses_outputs_over_its_inputs(over):
     # eight rows of 256 elements (q, out), nine of 128 (k, v)
     assert attention(**{**dict(q=A, k=C, v=D), **over}) == L.EINVAL
+    assert b"overlap" in L.load().idolq_last_error(), L.load().idolq_last_error()
+
+
+@pytest.mark.parametrize("over", [
+    dict(y=A), dict(y=A + 1024 + 1022), dict(y=A - 62), dict(y=B, ldy=24), dict(y=B, y_dtype=L.F32, ldy=16),
+    dict(y=B + 2), dict(y=B, y_dtype=L.F16, residual_dtype=L.BF16), dict(y=B - 32, y_dtype=L.BF16, ldy=32)])
+def test_q4_gemv_refuses_outputs_over_its_inputs(over):
+    # two rows of 512 (x) and of 16 elements (y, residual) in bf16
+    assert gemv(**{**dict(x=A, residual=B, residual_dtype=L.BF16, w=C, bias=D), **over}) == L.EINVAL
     assert b"overlap" in L.load().idolq_last_error(), L.load().idolq_last_error()
