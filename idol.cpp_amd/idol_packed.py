@@ -165,12 +165,15 @@ def _host_values(packed, kind, n, k):
     raise NotImplementedError(f"dequantize is not implemented for {GGMLQuantizationType(kind).name}")
 
 
-def enable_fused_packed(model, small_exact=False):
+def enable_fused_packed(model, small_exact=None):
     """Marks every PackedLinear of a fused kind for the fused path; returns how many (tools/idol_packed.py:85-94).
-    small_exact: calls of up to 16 rows of the 4-bit kinds read their blocks as they are (see PackedLinear)."""
+    small_exact: whether calls of up to 16 rows of the 4-bit kinds read their blocks as they are (see PackedLinear); None
+    leaves each layer as it is (off, unless an earlier call turned it on)."""
     layers = [m for m in model.modules() if isinstance(m, PackedLinear) and m.kind in _FUSED_KINDS]
     for layer in layers:
-        layer.fused, layer.small_exact = True, small_exact
+        layer.fused = True
+        if small_exact is not None:
+            layer.small_exact = bool(small_exact)
     return len(layers)
 
 

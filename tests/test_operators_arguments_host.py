@@ -1,8 +1,15 @@
 """Arguments of the packed attention, rotary and 4-bit product entry points on the host: sizes of workspaces, limits, and
-buffers that overlap. Every call below is refused before anything is launched (the pointers are never dereferenced)."""
+buffers that overlap; and the switch of the packed layers' exact small calls. Every call of the library below is refused
+before anything is launched (the pointers are never dereferenced)."""
+from types import SimpleNamespace
+
+import numpy as np
 import pytest
+import torch
 
 import idolq_lib as L
+from ggml_types import GGMLQuantizationType
+from idol_packed import PackedLinear, enable_fused_packed
 from test_operators_host import P, attention, gemv, rotary
 
 
@@ -57,3 +64,14 @@ def test_q4_gemv_refuses_outputs_over_its_inputs(over):
     # two rows of 512 (x) and of 16 elements (y, residual) in bf16
     assert gemv(**{**dict(x=A, residual=B, residual_dtype=L.BF16, w=C, bias=D), **over}) == L.EINVAL
     assert b"overlap" in L.load().idolq_last_error(), L.load().idolq_last_error()
+
+
+def test_enabling_the_fused_path_again_leaves_small_exact_as_it_is():
+    data = np.zeros((4, 2, 18), dtype=np.uint8)
+    net = torch.nn.Sequential(*(PackedLinear(SimpleNamespace(shape=np.array([64, 4]), tensor_type=GGMLQuantizationType.Q4_0,
+                                                             data=data), None) for _ in range(2)))
+    assert enable_fused_packed(net) == 2 and all(m.fused and not m.small_exact for m in net)
+    assert enable_fused_packed(net[1], small_exact=True) == 1
+    assert enable_fused_packed(net) == 2 and not net[0].small_exact and net[1].small_exact
+    enable_fused_packed(net, small_exact=False)
+    assert not any(m.small_exact for m in net)
