@@ -108,6 +108,8 @@ class PackedLinear(torch.nn.Module):
     def forward(self, value):
         if self._small(value):
             n, k = self.shape
+            if self.bias is not None and self.bias.dtype != value.dtype:  # as in the fused path's longer calls
+                raise ValueError('invalid fused linear bias')
             x = value.reshape(-1, k)
             if x.stride(-1) != 1 or (x.shape[0] > 1 and x.stride(0) < k):  # expanded rows too
                 x = x.contiguous()

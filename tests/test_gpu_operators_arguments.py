@@ -1,9 +1,14 @@
 """Views of one buffer that the packed attention, rotary and 4-bit product calls take as inputs and outputs, and those that
 they refuse because an output overlaps an input."""
+from types import SimpleNamespace
+
+import numpy as np
 import pytest
 import torch
 
 import idolq_lib as L
+from ggml_types import GGMLQuantizationType
+from idol_packed import PackedLinear, enable_fused_packed
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -62,3 +67,17 @@ def test_q4_gemv_into_its_residual_and_columns_next_to_its_inputs():
     for bad in (wide[:, 200:264], wide[:, 250:314], wide[:, 8:72]):
         with pytest.raises(ValueError, match="overlap"):
             call(out=bad)
+
+
+@pytest.mark.parametrize("rows_of_x", [3, 16, 17])
+def test_small_exact_calls_refuse_a_bias_of_another_type_as_longer_ones_do(rows_of_x):
+    data = np.zeros((8, 4, 18), dtype=np.uint8)
+    layer = PackedLinear(SimpleNamespace(shape=np.array([128, 8]), tensor_type=GGMLQuantizationType.Q4_0, data=data),
+                         torch.ones(8)).to(DEV)
+    enable_fused_packed(layer, small_exact=True)
+    x = rows(rows_of_x, 128, 6)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="invalid fused linear bias"):
+            layer(x)
+        layer.bias.data = layer.bias.data.to(BF16)
+        assert (layer(x) == 1).all()
