@@ -311,8 +311,8 @@ int idolq_q4_k_gemm(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ld
 
 /* y = epilogue(x * W^T) for m <= 16 activation rows on 4-bit weights as GGUF stores them, kind IDOLQ_KIND_Q4_0
  * (k % 32 == 0, 2-byte aligned) or IDOLQ_KIND_Q4_K (k % 256 == 0, 16-byte aligned): the weight bytes are read once,
- * 0.5625 a weight. x is bf16, fp16 or fp32 of any stride and alignment, with finite values (an infinite activation makes
- * its row NaN). EXACT arithmetic: the codes enter the products as they are and each group of 32 is scaled in fp32
+ * 0.5625 a weight. x is bf16, fp16 or fp32 of any stride and alignment, with magnitudes up to 2^117 (a group's products are
+ * summed before its scale; larger, infinite and NaN activations make their own row no number). n up to 2^27, k up to 2^24. EXACT arithmetic: the codes enter the products as they are and each group of 32 is scaled in fp32
  * (idolq_q8_0_gemm's and idolq_q4_k_gemm's DEQUANT rounds each weight to x's type first). bias, residual, act, y and the
  * flag IDOLQ_FLAG_ROUND_BEFORE_BIAS as idolq_q8_0_gemm; no workspace. The residual may be y itself (same stride and type);
  * y must not overlap it otherwise, nor x.
