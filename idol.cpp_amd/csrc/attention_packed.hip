@@ -1,8 +1,8 @@
 // Attention over packed sequences of different lengths, causal or not, with grouped heads, for gfx950.
 //
 // Sequence s holds the query rows [cu_q[s], cu_q[s + 1]) of q and the key rows [cu_k[s], cu_k[s + 1]) of k and v, or the
-// first k_lens[s] of these; query
-// head h reads key head h / (heads / kv_heads). Query i of lq sees the keys j < lk and, causal, j <= i + lk - lq:
+// first k_lens[s] of these; query head h reads key head h / (heads / kv_heads). Query i of lq sees the keys j < lk and,
+// causal, j <= i + lk - lq:
 //   o_i = sum_j 2^(u_ij - m_i) v_j / sum_j 2^(u_ij - m_i),  u_ij = scale log2(e) q_i . k_j,
 // for any m_i near the row's largest u; 0 where no key is left. The offsets are read on the device only (a captured graph
 // may be replayed with others) and clamped to the buffers' rows, so no offset reaches outside them; nothing on the host
@@ -16,8 +16,8 @@
 // transposed, S^T = K Q^T on the 32x32x16 matrix instructions, so a lane holds 32 scores of one row; the probabilities
 // become the B operand of O^T = V^T P^T from the registers they are in, and V^T is read out of the row-major V tile by
 // the transposing LDS reads in the key order that the scores have. m goes by the first tile's maximum and is raised only for
-// a tile with far larger scores. Tiles past a wave's last visible key are skipped, only tiles that some row
-// sees in part are masked. Bound by MFMAs and the softmax's vector work, of which little overlaps: one bf16 prompt of 16384,
+// a tile with far larger scores. Tiles past a wave's last visible key are skipped, only tiles that some row sees in part are
+// masked. Bound by MFMAs and the softmax's vector work, of which little overlaps: one bf16 prompt of 16384,
 // 32 heads on 8 of 128, 1.9 ms (1.1 PFLOP/s, matrix units busy 60% of the cycles), 8 fp16 prompts of up to 4096, 24 heads of
 // 64, 193 us (0.7; half the products for each exponential). Waves that take the next tile's scores among this tile's
 // exponentials were slower at both (2.1 ms, 221 us).
@@ -26,13 +26,13 @@
 // of a sequence's keys for all its rows; each of its waves walks its own 32-key tiles in LDS of its own, no barrier between
 // them, and the waves' (m, l, O) are merged through LDS. The chunks of all sequences are one list: chunk c of a sequence that
 // starts at key row b is entry b / chunk + s + c, so long and short sequences spread evenly; or, where that gives fewer
-// entries (lengths alike; caches mostly empty: 4 sequences of up to 4000 keys in 65536 rows each 28 us, with the list
-// 48), s per + c with per chunks for the longest. Parts of a sequence cut into several chunks go to the workspace in fp32 and
+// entries (lengths alike; caches mostly empty: 4 sequences of up to 4000 keys in 65536 rows each 21 us, with the list
+// 45), s per + c with per chunks for the longest. Parts of a sequence cut into several chunks go to the workspace in fp32 and
 // attn_packed_combine merges them in order.
 //
 // Probabilities are rounded to the inputs' type for the matrix product, and the sum l adds the rounded values, so the
-// weights still sum to 1. Each is off by up to 2^-9 (bf16) or 2^-12 (fp16) of itself, so an output by as much of
-// sum p_j |v_j| at most; over values of mean zero that is about what the output's own rounding is (48 sequences in bf16: 2.3e-3
+// weights still sum to 1. Each is off by up to u = 2^-9 (bf16) or 2^-12 (fp16) of itself, so an output by u (A + |o|) at most,
+// A = sum p_j |v_j|; over values of mean zero that is about what the output's own rounding is (48 sequences in bf16: 2.3e-3
 // of the result in all, 1.7e-3 with fp32 weights). Two bf16 parts a weight would take half as many matrix products again.
 // bf16: m lies 2^24 above the row's maximum, so that sums of values near the type's largest stay finite. fp16: 2^8 below it,
 // as small weights would vanish otherwise (a key 17.5 above 4096 others: a third of their weight).
@@ -366,8 +366,8 @@ struct RowLoader {
 
 // The parts first, first + step, .. of a row merged by 16 lanes (sub: which), HD / 16 columns each: entry(i) is part i's
 // unnormalized columns and its (m, l); parts without a sum (m = -inf) are left out, others keep what is no number in them
-// whatever their weight. Bound by the latency of its loads, so those of eight parts go together and the
-// maximum is a running one (48 sequences as below, the whole call: 128 us, with a pass for the maximum first 132).
+// whatever their weight. Bound by the latency of its loads, so those of eight parts go together and the maximum is a running
+// one (a pass for the maximum first: 4 us more for the call on 48 sequences below).
 template <int HD, typename F>
 __device__ __forceinline__ void merge_parts(const PackedParams& p, int first, int step, int parts, int sub, F&& entry,
                                             float (&o)[HD / 16], float& m, float& l) {
@@ -641,7 +641,7 @@ __device__ __forceinline__ int64_t first_part(const PackedParams& p, int s, int 
 }
 
 // NW waves: 4 for long key ranges, so that a CU holds two or three workgroups and one's loads, start and merge pass under the
-// others' work (48 sequences of up to 8192 keys, 32 heads on 8 of 128: 117 us in this kernel, 4.8 TB/s; one workgroup a CU
+// others' work (48 sequences of up to 8192 keys, 32 heads on 8 of 128: 113 us in this kernel, 4.9 TB/s; one workgroup a CU
 // whose waves load a tile ahead of their work into a second buffer 13 us more); as many as LDS holds for short ones, which
 // are then one or two tiles a wave and need no cutting, no workspace and no merge (500 keys, 16 heads of 64: 9.2 us, cut 2 us
 // more).

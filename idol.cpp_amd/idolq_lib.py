@@ -515,8 +515,9 @@ def attention_packed(q, k, v, cu_q, cu_k, heads, kv_heads, head_dim, causal=Fals
     projection buffers; cu_q and cu_k the sequences' first rows and the end, int32 [sequences + 1] on the device (not
     read here). k_lens, int32 [sequences] on the device: only the first k_lens[s] of a sequence's key rows count, so that a
     cache's sequences grow in place. Causal: query i of lq sees keys up to i + lk - lq. scale defaults to
-    1 / sqrt(head_dim). max_q and max_k, upper bounds of the query and key lengths, let the call choose its kernels and divide long key ranges well (0:
-    total_q, total_k). Rows of out outside every sequence are left as they were."""
+    1 / sqrt(head_dim). max_q and max_k, upper bounds of the query and key lengths, let the call choose its kernels and
+    divide long key ranges well (0: total_q, total_k). out must not overlap q, k or v; its rows outside every sequence are
+    left as they were."""
     lib = load()
     if heads < 1 or kv_heads < 1 or head_dim < 1:
         raise ValueError("heads, kv_heads and head_dim must be positive")
@@ -560,7 +561,7 @@ def rotary(x, heads, head_dim, positions, freqs, sections, k=None, kv_heads=0, i
     [rows, kv_heads * head_dim], turned by positions [rows, axes] (int32, int64 or fp32) times freqs (fp32, one per
     pair); sections holds each axis's pair count (their sum is freqs.numel(); elements behind the pairs are copied).
     Pairs are halves (j, j + P), or neighbours with interleaved=True; inverse=True turns back (also the gradient). Returns
-    the turned x, or (x, k); out and k_out may be x and k themselves."""
+    the turned x, or (x, k); out and k_out may be x and k themselves, other overlaps are refused."""
     lib = load()
     index = _device_index(x, k, positions, freqs, out, k_out)
     if x.dim() != 2 or positions.dim() != 2:

@@ -202,14 +202,16 @@ size_t idolq_attention_f32_workspace(int64_t batch, int64_t lq, int64_t lk, int6
  * k_lens[s] of these: a cache gives each sequence rows to grow into); query head h (columns
  * [h * head_dim, (h + 1) * head_dim) of q and out) reads key head h / (heads / kv_heads). Query i of lq sees the keys
  * j < lk and, causal, only j <= i + lk - lq (the last query sees every key); the softmax is over scale * (q . k). A query
- * that sees no key, or only keys with scores of -inf, gets zeros; what a masked key or value row holds (infinities and NaN too) does not reach the output; one
- * in a value row that a query sees with any score but -inf makes that column of the query no number (an infinity or NaN);
- * output rows outside every sequence are left as they were.
+ * that sees no key, or only keys with scores of -inf, gets zeros; what a masked key or value row holds (infinities and NaN
+ * too) does not reach the output; an infinity or NaN in a value row that a query sees with any score but -inf makes that
+ * column of the query one of the two; output rows outside every sequence are left as they were.
  *   dtype    IDOLQ_BF16 or IDOLQ_F16, of q, k, v and out; probabilities are rounded to it for their product with V (each off
  *            by up to 2^-9, fp16 2^-12, of itself; fp16 also by up to 2^-33 of the row's sum, which is more below 2^-22 of
  *            the largest), sums are fp32. head_dim 64 or 128; kv_heads divides heads.
  *   q, out   [total_q x heads * head_dim], row strides ldq, ldo; k, v [total_k x kv_heads * head_dim], row strides ldk,
- *            ldv; all 16-byte aligned in address and row stride. out must not overlap the inputs.
+ *            ldv; all 16-byte aligned in address and row stride, ldk and ldv up to 2^24. out must not overlap the inputs
+ *            (columns of one buffer may hold both). Rows below 2^31, heads up to 4096, seqs below 2^20, and
+ *            (total_q * heads / kv_heads / 128 + seqs) * kv_heads below 2^23.
  *   cu_q, cu_k  seqs + 1 device int32 each, not decreasing. They are read by the kernels only, so a captured call may be
  *            replayed with other lengths; values outside [0, total_q] or [0, total_k] are clamped to it.
  *   k_lens   seqs device int32 (clamped to 0 and the sequence's rows), or null: all rows. Rows behind are not read.
@@ -217,14 +219,14 @@ size_t idolq_attention_f32_workspace(int64_t batch, int64_t lq, int64_t lk, int6
  *            total_q, total_k); longer sequences are computed correctly too, only slower
  *   workspace  idolq_attention_packed_workspace() bytes (16-byte aligned, no zero-fill) let a call with few queries
  *            divide long key ranges over the device; without it (null or short) each query's keys stay with one
- *            workgroup. Calls sharing a workspace must not overlap.
+ *            workgroup. The parts of prompts' rows take up to 270 MB, those of few queries up to 64 rows for each of
+ *            2048 + kv_heads chunks (or 64 MB if that is more). Calls sharing a workspace must not overlap.
  * The fused form of src/kernels.hpp:81-84 attention for a batch of sequences; the reference has no mask and one length. */
 int idolq_attention_packed(const void* q, const void* k, const void* v, int dtype, int64_t seqs, const int32_t* cu_q,
                            const int32_t* cu_k, const int32_t* k_lens, int64_t total_q, int64_t total_k, int64_t max_q,
-                           int64_t max_k,
-                           int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t ldq, int64_t ldk, int64_t ldv,
-                           float scale, int causal, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
-                           void* stream);
+                           int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t ldq, int64_t ldk,
+                           int64_t ldv, float scale, int causal, void* out, int64_t ldo, void* workspace,
+                           size_t workspace_bytes, void* stream);
 size_t idolq_attention_packed_workspace(int64_t seqs, int64_t total_q, int64_t total_k, int64_t max_q, int64_t max_k,
                                         int64_t heads, int64_t kv_heads, int64_t head_dim);
 
@@ -240,6 +242,7 @@ enum { IDOLQ_ROTARY_INTERLEAVED = 1, IDOLQ_ROTARY_INVERSE = 2 };
  *   x, y     [rows x heads * head_dim], row strides ldx, ldy; y may be x (same stride), else they must not overlap
  *   x2, y2   a second tensor turned by the same positions (the keys) in the same launch; heads2 = 0 for none. y2 may be x2;
  *            other overlaps of an output with an input or the other output are refused
+ *   rows     below 2^24 are always taken (more where a workgroup holds several); heads and heads2 up to 65535
  *   head_dim 2 to 256; any strides and alignment (16-byte accesses where addresses, strides and sections allow them)
  *   pos      [rows x axes] of pos_kind IDOLQ_POS_I32, IDOLQ_POS_I64 or IDOLQ_POS_F32, row stride ldp; freqs [P] fp32
  * The angle is formed and reduced in fp64, so far positions keep fp32's accuracy.
