@@ -139,6 +139,9 @@ struct Prob<__bf16> {
     static constexpr float kBias = 24.0f;   // m lies this far above the maximum (fp32 sums of large values stay finite)
     static constexpr float kRise = 8.0f;    // a row whose largest score would move m further up than this does so
     static constexpr float kMost = 0x1p-9f;  // for a lane's sum of a tile that reaches this
+    // Below this m, rounded in fp32, lies so near its place that keys with the largest score do not reach kMost: half a step
+    // is 8 at most, 32 weights 2^(-24 + 8 + 5). Further out m might not move while o and l are scaled, tile by tile.
+    static constexpr float kFar = 0x1p28f;
     static __device__ __forceinline__ float sum(bf16x2 a, float c) {
         return __builtin_amdgcn_fdot2_f32_bf16(a, bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
     }
@@ -150,6 +153,7 @@ struct Prob<_Float16> {
     static constexpr float kBias = -8.0f;
     static constexpr float kRise = 0.0f;
     static constexpr float kMost = 0x1p15f;
+    static constexpr float kFar = 0x1p24f;  // half a step 1/2, 32 weights 2^(8 + 1/2 + 5)
     static __device__ __forceinline__ float sum(f16x2 a, float c) {
         return __builtin_amdgcn_fdot2(a, f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
     }
@@ -278,10 +282,10 @@ struct WaveRows {
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[st][r]);
             return fmaxf(mx, __shfl_xor(mx, 32));
         };
-        // Where a row's reference point goes from m: kBias above its largest score, which lies mx above m. Scores of 2^20 and
-        // more are their own reference point: in fp32 it would not move by kBias, and o and l would lose 2^-24 every tile.
+        // Where a row's reference point goes from m: kBias above its largest score, which lies mx above m. Scores of kFar and
+        // more are their own reference point.
         auto raise_to = [&](float mx) __attribute__((always_inline)) {
-            return mx + (fabsf(m + mx) < 0x1p20f ? Prob<T>::kBias : 0.0f);
+            return mx + (fabsf(m + mx) < Prob<T>::kFar ? Prob<T>::kBias : 0.0f);
         };
         auto lower = [&](float by) __attribute__((always_inline)) {
             m += by;

@@ -39,6 +39,18 @@ def test_large_scores_that_tie(way, power, dtype):
 
 
 @pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("power", [3, 19, 22, 25, 27])
+def test_large_scores_that_tie_over_values_near_the_largest(way, power):
+    # bf16 sums stay finite: hundreds of values of an eighth of the largest with the same weight
+    lq, lk = WAYS[way][:2]
+    q, k, v = torch.zeros((lq, 64)), torch.zeros((lk, 64)), 1 + rows(lk, 64, 11, 0.1).clamp(-0.5, 0.5)
+    q[:, 3], k[:, 3] = 2.0 ** 10, 2.0 ** 10
+    q, k, v = q.to(BF16).to(DEV), k.to(BF16).to(DEV), (v * (torch.finfo(BF16).max / 8)).to(BF16).to(DEV)
+    want = v.double().cpu().mean(0).expand(lq, 64)
+    check(call(q, k, v, way, scale=2.0 ** (power - 20)), want, want, BF16)
+
+
+@pytest.mark.parametrize("way", list(WAYS))
 @pytest.mark.parametrize("gap", [12.0, 15.0, 17.5, 19.0])
 @pytest.mark.parametrize("dtype,hd", [(FP16, 64), (FP16, 128), (BF16, 64)])
 def test_small_weights_next_to_a_dominant_key(way, gap, dtype, hd):
