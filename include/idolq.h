@@ -207,7 +207,8 @@ size_t idolq_attention_f32_workspace(int64_t batch, int64_t lq, int64_t lk, int6
  * column of the query one of the two; output rows outside every sequence are left as they were.
  *   dtype    IDOLQ_BF16 or IDOLQ_F16, of q, k, v and out; probabilities are rounded to it for their product with V (each off
  *            by up to 2^-9, fp16 2^-12, of itself; fp16 also by up to 2^-33 of the row's sum, which is more below 2^-22 of
- *            the largest), sums are fp32. head_dim 64 or 128; kv_heads divides heads.
+ *            the largest), sums are fp32 (bf16: of weights 2^-24 times theirs, so that values near the largest do not
+ *            overflow; values below 2^-100 lose bits). head_dim 64 or 128; kv_heads divides heads.
  *   q, out   [total_q x heads * head_dim], row strides ldq, ldo; k, v [total_k x kv_heads * head_dim], row strides ldk,
  *            ldv; all 16-byte aligned in address and row stride, ldk and ldv up to 2^24. out must not overlap the inputs
  *            (columns of one buffer may hold both). Rows below 2^31, heads up to 4096, seqs below 2^20, and
